@@ -1,0 +1,39 @@
+"""What the native sources must not hold, read from their text: instructions that have proved unsafe on the hardware, in probes that
+nothing builds and in comments as much as in kernels.  The patterns are spelt so that this file does not match them."""
+import os
+import re
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+FOLDERS = ("crispresso2_amd", "include", "oracle", "tests", "tools")
+SUFFIXES = (".hip", ".h", ".hpp", ".c", ".cc", ".cpp", ".s", ".S", ".py", ".sh", ".mk")
+NAMES = ("Makefile", "CMakeLists.txt")
+SKIPPED = ("__pycache__", "lib", "_ref", "golden", "build")          # built files and recorded data
+
+
+def sources():
+    found = [os.path.join(ROOT, n) for n in os.listdir(ROOT)]
+    for folder in FOLDERS:
+        for d, subs, names in os.walk(os.path.join(ROOT, folder)):
+            subs[:] = [x for x in subs if x not in SKIPPED]
+            found += [os.path.join(d, n) for n in names]
+    return sorted(f for f in found if os.path.isfile(f) and (f.endswith(SUFFIXES) or os.path.basename(f) in NAMES))
+
+
+def lines_with(pattern):
+    rx = re.compile(pattern)
+    out = []
+    for f in sources():
+        with open(f, encoding="utf-8", errors="replace") as fh:
+            out += ["%s:%d: %s" % (os.path.relpath(f, ROOT), k, m.group(0)) for k, line in enumerate(fh, 1) for m in [rx.search(line)] if m]
+    return out
+
+
+def test_the_walk_reaches_every_kind_of_source():
+    got = {os.path.relpath(f, ROOT) for f in sources()}
+    assert {"bench.py", "crispresso2_amd/csrc/Makefile", "crispresso2_amd/csrc/c2_k_align.hip", "crispresso2_amd/csrc/c2_fastq.cpp",
+            "include/crispresso2_amd.h", "oracle/c2_oracle.c", "tests/emu/emu_harness.cpp", "tools/build_variant.sh"} <= got
+
+
+def test_nothing_writes_through_the_scalar_data_cache():
+    """Scalar stores, scalar atomics, and the scalar data cache's write-back and discard: data is written by vector stores."""
+    assert lines_with(r"\bs_(?:[a-z0-9]+_)*(?:store|atomic|dcache)(?:_[a-z0-9]+)*") == []
