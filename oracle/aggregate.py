@@ -13,7 +13,8 @@ import numpy as np
 
 def aggregate(items, ref_len, ignore_substitutions=False, ignore_insertions=False, ignore_deletions=False,
               discard_indel_reads=False):
-    """items: iterable of (payload dict incl. 'aln_seq', count)."""
+    """items: iterable of (payload dict incl. 'aln_seq', count).  Substituted bases: letters (the reference's payload) or byte codes (the
+    classifier kernels' flat lists)."""
     L = ref_len
     v = {k: np.zeros(L) for k in (
         "all_insertion_count_vectors", "all_insertion_left_count_vectors", "all_deletion_count_vectors",
@@ -74,7 +75,7 @@ def aggregate(items, ref_len, ignore_substitutions=False, ignore_insertions=Fals
                 s["counts_substitution"] += count
                 has_sub = True
             for nuc in "ATCGN":                                                          # :4048-4054
-                locs = [q for q, b in zip(p["all_substitution_positions"], p["all_substitution_values"]) if b == nuc]
+                locs = [q for q, b in zip(p["all_substitution_positions"], p["all_substitution_values"]) if b in (nuc, ord(nuc))]
                 if locs:
                     v["all_substitution_base_vectors_" + nuc][locs] += count
         if has_del:                                                                      # :4058-4072

@@ -134,3 +134,29 @@ def test_oracle_live_fuzz_against_reference(mats):
         inc = list(range(int(rng.integers(0, L)), L))[: int(rng.integers(1, 20))]
         assert payload_diff(oracle.find_indels_substitutions(got[0], got[1], inc),
                             R.find_indels_substitutions(exp[0], exp[1], inc).__dict__) == []
+
+
+@pytest.mark.parametrize("codes", [list, np.array])
+def test_aggregate_takes_substituted_bases_as_letters_or_byte_codes(codes):
+    """The reference's payload spells a substituted base as a letter, the classifier kernels' flat lists hold its byte code: the same
+    vectors from both, against counts written out by hand (an N in the read is no substitution, COREResources.pyx:113)."""
+    from oracle import aggregate
+    amp = "ACGTACGTAC"
+    reads = [("TCGTACGTAC", 3), ("ACGNACGTAA", 5), ("ACCTACGTAG", 7)]
+    letters, flat = [], []
+    for s1, c in reads:
+        p = oracle.find_indels_substitutions(s1, amp, [2, 3])
+        p["aln_seq"], p["aln_ref"] = s1, amp
+        assert all(isinstance(b, str) for b in p["all_substitution_values"])
+        letters.append((p, c))
+        q = dict(p)
+        for k in ("all_substitution_values", "substitution_values"):
+            q[k] = codes([ord(b) for b in p[k]])
+        flat.append((q, c))
+    want = {"T": {0: 3}, "N": {}, "A": {9: 5}, "C": {2: 7}, "G": {9: 7}}
+    for items in (letters, flat):
+        got = aggregate.aggregate(items, len(amp))
+        for n in "ACGTN":
+            assert {int(k): int(got["all_substitution_base_vectors_" + n][k]) for k in np.flatnonzero(got["all_substitution_base_vectors_" + n])} == want[n]
+    a, b = aggregate.aggregate(letters, len(amp)), aggregate.aggregate(flat, len(amp))
+    assert a.keys() == b.keys() and all(np.array_equal(a[k], b[k]) for k in a)
