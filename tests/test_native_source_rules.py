@@ -2,6 +2,7 @@
 nothing builds and in comments as much as in kernels.  The patterns are spelt so that this file does not match them."""
 import os
 import re
+import subprocess
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 FOLDERS = ("crispresso2_amd", "include", "oracle", "tests", "tools")
@@ -42,3 +43,23 @@ def test_nothing_writes_through_the_scalar_data_cache():
 def test_no_source_writes_packed_fp32_arithmetic():
     """The two-wide float add, multiply and multiply-add: some of their forms give wrong results now and then, without an error."""
     assert lines_with(r"\bv_pk_(?:add|mul|fma)_f32") == []
+
+
+PACKED_FP32_OFF = "-Xclang -target-feature -Xclang -packed-fp32-ops"
+
+
+def test_every_unit_is_compiled_with_packed_fp32_off():
+    """The compiler makes packed FP32 from ordinary float code by itself unless it is told not to: every compile line of the library,
+    of the A/B builds, and the build line of each probe."""
+    out = subprocess.run(["make", "-n", "-B", "-C", os.path.join(ROOT, "crispresso2_amd", "csrc"), "HIPCC=hipcc"],
+                         check=True, capture_output=True, text=True).stdout
+    compiles = [x for x in out.splitlines() if x.startswith("hipcc") and " -c " in x]
+    units = [re.search(r" -c (\S+) -o \.\./lib/obj/(\S+)\.o$", x).groups() for x in compiles]
+    assert len(units) == 6 and all(src in (obj + ".hip", obj + ".cpp") for src, obj in units)
+    assert all(PACKED_FP32_OFF in x for x in compiles)
+    lines = []
+    for f in sources():
+        if f.endswith((".sh", ".hip")):
+            with open(f, encoding="utf-8") as fh:
+                lines += [x for x in fh if "hipcc " in x and "--offload-arch" in x and ".hip" in x]
+    assert lines and all(PACKED_FP32_OFF in x for x in lines)

@@ -8,7 +8,7 @@ ROOT=$(cd "$(dirname "$0")/.." && pwd)
 cd "$ROOT/crispresso2_amd/csrc"
 make -j8 >/dev/null
 mkdir -p ../lib/variants ../lib/obj_variants
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -I. -I../../include $FLAGS -c $UNIT.hip -o ../lib/obj_variants/${UNIT}_$NAME.o
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Xclang -target-feature -Xclang -packed-fp32-ops -I. -I../../include $FLAGS -c $UNIT.hip -o ../lib/obj_variants/${UNIT}_$NAME.o
 OBJS=$(ls ../lib/obj/*.o | grep -v "/$UNIT.o")
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC $OBJS ../lib/obj_variants/${UNIT}_$NAME.o -lz -lpthread -o ../lib/variants/lib_$NAME.so
 echo "../lib/variants/lib_$NAME.so"
