@@ -63,3 +63,26 @@ def test_every_unit_is_compiled_with_packed_fp32_off():
             with open(f, encoding="utf-8") as fh:
                 lines += [x for x in fh if "hipcc " in x and "--offload-arch" in x and ".hip" in x]
     assert lines and all(PACKED_FP32_OFF in x for x in lines)
+
+
+def test_build_compiles_also_where_a_library_is_there(monkeypatch):
+    """File times cannot say whether a built library belongs to the sources beside it (a copied tree, a changed compiler or variable):
+    build() asks make for every unit."""
+    import __graft_entry__ as entry
+
+    class Stop(Exception):
+        pass
+
+    asked = []
+
+    def check_call(cmd, *a, **k):
+        asked.append(cmd)
+        raise Stop
+    monkeypatch.setattr(entry.subprocess, "check_call", check_call)
+    try:
+        entry.build()
+    except Stop:
+        pass
+    assert len(asked) == 1 and asked[0][0] == "make"
+    out = subprocess.run(asked[0] + ["-n"], check=True, capture_output=True, text=True).stdout
+    assert len([x for x in out.splitlines() if " -c " in x]) == 6
